@@ -11,7 +11,6 @@ Three kinds of operator, in the order in which a token row meets them:
 
 A case holds plain values; the layers' sizes are those of the repository's configurations (7168 x 2048, 4096, 5120) and odd ones.
 """
-import functools
 import math
 import sys
 from pathlib import Path
@@ -26,7 +25,6 @@ _TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32, 
 _BYTES = {"bf16": 2, "fp16": 2, "fp32": 4, "fp8": 1}
 
 
-@functools.lru_cache(maxsize=None)
 def _package():
     for p in (Path.cwd() / "flaggems-sglang_b200", _ROOT / "flaggems-sglang_b200"):
         if p.is_dir():
