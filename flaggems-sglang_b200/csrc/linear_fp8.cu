@@ -61,7 +61,8 @@ linear_quant_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict_
   for (int u = 0; u < kQuantRuns; ++u) {
     const int g = g0 + u * halves, e0 = g * kSlice + l16 * 8;
     const float s = group_scale(m[u]);
-    store_q8<true>(q + row * K + e0, e0 < K ? 8 : 0, e4m3_divided(v[u], s));
+    // (the division's own reciprocal: with divisor_of's the compiler takes the groups one after the other, 0.6 us more for 48 rows of 2048)
+    store_q8<true>(q + row * K + e0, e0 < K ? 8 : 0, e4m3_divided(v[u], divisor_of(s, __frcp_rn(s))));
     if (l16 == 0 && g < G) scales[row * G + g] = s;
   }
 }
@@ -306,7 +307,7 @@ fp8_linear_decode_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
 #pragma unroll
       for (int u = 0; u < kOwnGroups; ++u) {
         const float s = group_scale(m[u]);
-        const uint2 q = e4m3_divided(v[u], s);
+        const uint2 q = e4m3_divided(v[u], divisor_of(s));
         if (xt[u] < live) {
           *reinterpret_cast<uint2*>(s_x + xi[u] * kFusedSlice + xt[u] * kSlice + (((l16 >> 1) ^ xt[u]) << 4) + (l16 & 1) * 8) = q;
           if (l16 == 0) s_t[xi[u] * NT + xt[u]] = s * ws[xi[u]];

@@ -486,7 +486,7 @@ block_norm_stream_kernel(const NormArgs a, int stages, int stage_bytes) {
         }
         const float sc = group_scale(max16(amax8(y)));     // (zeros beyond the row)
         if (!FAST && !there[c]) continue;
-        store_q8<true>(py + c * hop, 8, e4m3_scaled(v[c], group_reciprocal(sc)));
+        store_q8<true>(py + c * hop, 8, e4m3_divided(v[c], divisor_of(sc)));
         if ((lane & 15) == 0) ps[c * (hop >> 7)] = sc;
       }
       py += step_y;

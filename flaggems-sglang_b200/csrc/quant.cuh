@@ -6,17 +6,12 @@ namespace b200moe {
 
 // A group's scale: max(amax, 1e-10) / 448 (what per_token_group_quant_fp8 stores).  The divisor is known: the product with its
 // reciprocal, corrected once by the exact remainder (Brisebarre, Muller and Raina, "Accelerating correctly rounded floating-point division when
-// the divisor is known in advance", 2004).  Compared with __fdiv_rn for every float from 1e-10 to infinity.
+// the divisor is known in advance", 2004).  Compared with a division for every mantissa, at both ends of
+// the range too.
 __device__ __forceinline__ float group_scale(float amax) {
   const float x = fmaxf(amax, 1e-10f), q = x * (1.0f / 448.0f);
   return x < INFINITY ? fmaf(fmaf(-448.0f, q, x), 1.0f / 448.0f, q) : x;
 }
-// 1 / s, within 2^-23 of it: an approximate reciprocal and one step of Newton's iteration.
-__device__ __forceinline__ float group_reciprocal(float s) {
-  const float r = __fdividef(1.0f, s);
-  return s < INFINITY ? fmaf(r, fmaf(-s, r, 1.0f), r) : 0.f;
-}
-
 __device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
   unsigned long long r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -36,45 +31,37 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
 
-// Eight values times the reciprocal of their group's scale, rounded to nearest even and saturated.
-__device__ __forceinline__ uint2 e4m3_scaled(const float (&v)[8], float inv) {
-  uint32_t q[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) q[i] = e4m3x2(v[2 * i] * inv, v[2 * i + 1] * inv);
-  return make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
+// e4m3(v / s), the quotient as an IEEE division rounds it (but for a negative zero, which comes out positive): the product with the
+// reciprocal, corrected by the quotient's exact remainder (Markstein, "Computation of elementary functions on the IBM RISC
+// System/6000 processor", 1990).  The reciprocal is the correctly rounded one: an approximate one and a step of Newton's iteration, compared
+// with __frcp_rn for every mantissa.  An infinite scale divides every number to zero and infinities to NaN.  The product alone is off by up to
+// 1.5 ulp, with the same error of the reciprocal for a whole group, which moved values of the norms and the activation over boundaries of e4m3;
+// and 16-bit values over a scale of their own are ties so often (every second warp held one) that redoing the division where the
+// product lies next to a boundary doubled the kernel's instructions.
+struct Divisor {
+  unsigned long long inv2, neg2;
+};
+__device__ __forceinline__ Divisor divisor_of(float s, float inv) {
+  const float neg = s < INFINITY ? -s : 0.f;
+  return {pack_f32x2(inv, inv), pack_f32x2(neg, neg)};
 }
-__device__ __forceinline__ uint2 e4m3_scaled(const unsigned long long (&v)[4], float inv) {
-  const unsigned long long inv2 = pack_f32x2(inv, inv);
-  uint32_t q[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float a, b;
-    unpack_f32x2(mul2(v[i], inv2), a, b);
-    q[i] = e4m3x2(a, b);
-  }
-  return make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
+__device__ __forceinline__ Divisor divisor_of(float s) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+  return divisor_of(s, s < INFINITY ? fmaf(r, fmaf(-s, r, 1.0f), r) : 0.f);
 }
-// For values that are themselves results of fp32 arithmetic: v * (1 / s).  (Without the step of Newton's iteration the error of 1 / s,
-// the same for a whole group, moved twice as many values over a boundary.)
-__device__ __forceinline__ uint2 e4m3_of8(const float (&v)[8], float s) { return e4m3_scaled(v, group_reciprocal(s)); }
-
-// The bits of e4m3(v / s) with an IEEE division (compared for every 16-bit value over the scale of every 16-bit maximum; a negative zero comes
-// out positive), without eight of them: the product with the correctly rounded reciprocal, corrected by the
-// quotient's exact remainder (Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor", 1990).
-// 16-bit values over a scale of their own are ties so often (every second warp held one) that redoing the division where the product lies
-// next to a boundary doubled the kernel's instructions.
-__device__ __forceinline__ uint2 e4m3_divided(const float (&v)[8], float s) {
-  const float inv = __frcp_rn(s);
-  const unsigned long long inv2 = pack_f32x2(inv, inv), neg2 = pack_f32x2(-s, -s);
-  uint32_t q[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const unsigned long long v2 = pack_f32x2(v[2 * i], v[2 * i + 1]), r = mul2(v2, inv2);
-    float a, b;
-    unpack_f32x2(fma2(fma2(neg2, r, v2), inv2, r), a, b);
-    q[i] = e4m3x2(a, b);
-  }
-  return make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
+__device__ __forceinline__ uint32_t e4m3_pair(unsigned long long v2, const Divisor& d) {
+  const unsigned long long r = mul2(v2, d.inv2);
+  float a, b;
+  unpack_f32x2(fma2(fma2(d.neg2, r, v2), d.inv2, r), a, b);
+  return e4m3x2(a, b);
+}
+__device__ __forceinline__ uint2 e4m3_divided(const unsigned long long (&v)[4], const Divisor& d) {
+  return make_uint2(e4m3_pair(v[0], d) | e4m3_pair(v[1], d) << 16, e4m3_pair(v[2], d) | e4m3_pair(v[3], d) << 16);
+}
+__device__ __forceinline__ uint2 e4m3_divided(const float (&v)[8], const Divisor& d) {
+  const unsigned long long v2[4] = {pack_f32x2(v[0], v[1]), pack_f32x2(v[2], v[3]), pack_f32x2(v[4], v[5]), pack_f32x2(v[6], v[7])};
+  return e4m3_divided(v2, d);
 }
 
 __device__ __forceinline__ float amax8(const float (&v)[8]) {
@@ -187,7 +174,7 @@ template <bool VEC>
 __device__ __forceinline__ void quantise8(const float (&v)[8], uint8_t* q, float* scale, int e0, int n, int lane) {
   if (VEC) {
     const float s = group_scale(max16(amax8(v)));
-    store_q8<true>(q + e0, n, e4m3_of8(v, s));
+    store_q8<true>(q + e0, n, e4m3_divided(v, divisor_of(s)));
     if ((lane & 15) == 0 && n > 0) scale[e0 >> 7] = s;
   } else {
     float m[2] = {0.f, 0.f};
@@ -199,7 +186,7 @@ __device__ __forceinline__ void quantise8(const float (&v)[8], uint8_t* q, float
       m[1] = fmaxf(m[1], __shfl_xor_sync(0xffffffffu, m[1], o));
     }
     const float s0 = group_scale(m[0]), s1 = group_scale(m[1]);
-    store_q8<false>(q + e0, n, make_uint2(e4m3_of8(v, s0).x, e4m3_of8(v, s1).y));
+    store_q8<false>(q + e0, n, make_uint2(e4m3_divided(v, divisor_of(s0)).x, e4m3_divided(v, divisor_of(s1)).y));
     if (lane == 0 && n > 0) scale[e0 >> 7] = s0;
     if (lane == 0 && n > 4) scale[(e0 >> 7) + 1] = s1;
   }
