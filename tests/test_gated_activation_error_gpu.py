@@ -56,3 +56,27 @@ def test_silu_at_the_ends(cuda_device):
     y = F.gated_activation(torch.cat([g, one], 1))[0].tolist()
     assert y[0] == inf and y[1] != y[1] and y[2] != y[2] and y[3] == float(g[0, 3]) and y[4] == 0 and y[5] == 0 and y[6] == 0
     assert y[7] == 200 and y[8] == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lo,hi", [(-1, 1), (-4, 4), (-13, -4), (-40, 40)])
+def test_gelu(cuda_device, dtype, lo, hi):
+    """Units of 2^-24: the fitted polynomial and its roundings 7, the reciprocal 2, which the function turns into at most 2.3 times as many,
+    the exponential 5, three products 3: 20, below 2^-19, of the result, in the tail too.  16-bit rows: two roundings of g^2 / 2 more.  Then
+    half a step of the type."""
+    import flaggems_sglang_b200 as F
+    g, u = rows(cuda_device, lo, hi)
+    x = torch.cat([g, u], 1).to(dtype)
+    g, u = x.double().chunk(2, 1)
+    want = g * (0.5 * torch.special.erfc(-g * 0.5 ** 0.5)) * u
+    half, least = (0, 2.0 ** -126) if dtype == torch.float32 else (torch.finfo(dtype).eps / 2, 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -126)
+    relative(F.gated_activation(x, "gelu"), want, 2.0 ** -19 + half + (2.0 ** -24 * g.square() if half else 0), least + 2.0 ** -126 * (g * u).abs())
+
+
+def test_gelu_at_the_ends(cuda_device):
+    import flaggems_sglang_b200 as F
+    inf, nan = float("inf"), float("nan")
+    g = torch.tensor([[inf, -inf, nan, 3e38, -3e38, 0.0, -0.0, 20.0, -20.0]], device=cuda_device)
+    y = F.gated_activation(torch.cat([g, torch.ones_like(g)], 1), "gelu")[0].tolist()
+    assert y[0] == inf and y[1] != y[1] and y[2] != y[2] and y[3] == float(g[0, 3]) and y[4] == 0 and y[5] == 0 and y[6] == 0
+    assert y[7] == 20 and y[8] == 0
