@@ -7,7 +7,8 @@
 //
 // Everything between the loads and the stores is fp32; h and y are each rounded once, y from the h that was not yet rounded.
 // A row is read once: its elements stay in registers over both norms, eight to a chunk, CH chunks to a thread, `team` threads to a
-// row.  Variances are taken around the mean in a second pass over the registers, so rows with a large mean lose nothing.
+// row.  Variances are taken around the mean in a second pass over the registers, and what the
+// mean's own rounding left there is taken off both, so rows with a large mean lose nothing.
 // Sums: shuffles within a warp, then one exchange through shared memory, always in the same order.
 //
 // Bound by HBM where there are many rows (of a copy's 6.54 TB/s): before a block, 4096 x 7168 quantised, 206.5 MB in 35.0 us, 90 %; after
@@ -15,6 +16,7 @@
 // rows through four round trips of sums and reach 60 % (4096 x 4096, quantised, 30.2 us).  By a launch and one round trip to memory where
 // there are few: one row of 7168 in 2.6 us, 33 of 4096 with both norms in 3.2.
 #include <algorithm>
+#include <type_traits>
 
 #include "block_ops.cuh"
 #include "quant.cuh"
@@ -24,7 +26,8 @@ namespace b200moe {
 namespace {
 
 constexpr int kRingBytes = 220 * 1024, kSmBytes = 226 * 1024;     // shared memory of a CTA's ring, of an SM's
-constexpr int kMaxSums = 4;     // a row's block-wide sums: mean and variance of two norms
+constexpr int kNormSums = 3;    // block-wide sums of a norm of one row: the mean; the mean of the differences from it, and their squares
+
 
 // Sum over the row's team.  `s`: one slot per warp of the CTA, used once.
 __device__ __forceinline__ float team_sum(float v, float* s, int warps, int warp0, int lane) {
@@ -37,6 +40,34 @@ __device__ __forceinline__ float team_sum(float v, float* s, int warps, int warp
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
+}
+
+// Two sums in the shuffles of one: after the first of them a half warp carries each.  `s`: `slots` apart.
+__device__ __forceinline__ void team_sum(float& a, float& b, float* s, int slots, int warps, int warp0, int lane) {
+  const bool upper = (lane & 16) != 0;
+  float v = (upper ? b : a) + __shfl_xor_sync(0xffffffffu, upper ? a : b, 16);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (warps > 1) {
+    float* mine = s + (upper ? slots : 0);
+    const int l = lane & 15;
+    if (l == 0) mine[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = l < warps ? mine[warp0 + l] : 0.f;
+    if (l + 16 < warps) v += mine[warp0 + l + 16];
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  }
+  const float other = __shfl_xor_sync(0xffffffffu, v, 16);
+  a = upper ? other : v;
+  b = upper ? v : other;
+}
+
+// A layer norm's mean is off by some roundings of itself, which can be many times the deviation where rows are nearly constant.  So the
+// differences' own mean `d` is summed beside their squares and taken off both: of equal elements nothing is left.
+__device__ __forceinline__ float variance(float squares, float d) {
+  const float v = fmaf(-d, d, squares);
+  return v < 0.f ? 0.f : v;
 }
 
 // Weights, biases and per-channel gates come in the rows' type or in fp32.
@@ -67,17 +98,18 @@ __device__ __forceinline__ float chunk_sum(const float (&v)[CH][8]) {
 
 // v = norm(v); elements beyond the row (n[c] of eight are there) are zero on entry and left as they come out
 // EARLY: the weights are on their way during the sums (few rows, where that is a round trip); else they are read where they are used
-template <typename T, bool VEC, int CH, bool EARLY>
+template <typename T, bool VEC, int CH, bool EARLY, bool LAYER>
 __device__ __forceinline__ void normalise(float (&v)[CH][8], const int (&n)[CH], const int (&e0)[CH], const NormArgs& a,
-                                          const void* w, const void* b, bool w_f32, bool b_f32, float* s0, float* s1, int warps,
+                                          const void* w, const void* b, bool w_f32, bool b_f32, float* sums, int slots, int warps,
                                           int warp0, int lane) {
   Vector8<T> wr[EARLY ? CH : 1];
   if (EARLY && w != nullptr) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) load_vector<T, VEC>(w, w_f32, e0[c], n[c], wr[c]);
   }
-  if (a.layer) {
-    const float mean = team_sum(chunk_sum<CH>(v), s0, warps, warp0, lane) / static_cast<float>(a.H);
+  const float h = static_cast<float>(a.H);
+  if (LAYER) {
+    const float mean = team_sum(chunk_sum<CH>(v), sums, warps, warp0, lane) / h;
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
@@ -88,18 +120,26 @@ __device__ __forceinline__ void normalise(float (&v)[CH][8], const int (&n)[CH],
   for (int c = 0; c < CH; ++c)
 #pragma unroll
     for (int i = 0; i < 8; ++i) q = fmaf(v[c][i], v[c][i], q);
-  const float r = rsqrtf(team_sum(q, s1, warps, warp0, lane) / static_cast<float>(a.H) + a.eps);
+  float r, shift = 0.f;
+  if (LAYER) {
+    float d = chunk_sum<CH>(v);
+    team_sum(d, q, sums + slots, slots, warps, warp0, lane);
+    d /= h;
+    r = rsqrtf(variance(q / h, d) + a.eps);
+    shift = -d * r;
+  } else {
+    r = rsqrtf(team_sum(q, sums, warps, warp0, lane) / h + a.eps);
+  }
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[c][i] = LAYER ? fmaf(v[c][i], r, (VEC ? n[c] > 0 : i < n[c]) ? shift : 0.f) : v[c][i] * r;
     if (w != nullptr) {
       float f[8];
       if (!EARLY) load_vector<T, VEC>(w, w_f32, e0[c], n[c], wr[0]);
       unpack_vector<T>(wr[EARLY ? c : 0], w_f32, f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[c][i] = v[c][i] * r * (a.offset + f[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[c][i] *= r;
+      for (int i = 0; i < 8; ++i) v[c][i] *= a.offset + f[i];
     }
     if (b != nullptr) {
       Vector8<T> br;
@@ -122,15 +162,15 @@ __device__ __forceinline__ void load_gate_chunk(const NormArgs& a, long long row
 }
 
 // A row from its loaded elements to its stores.
-template <typename T, typename R, bool VEC, int CH, bool EARLY, bool POST = true, bool PRE = true>
+template <typename T, typename R, bool VEC, int CH, bool EARLY, bool LAYER, bool POST = true, bool PRE = true>
 __device__ __forceinline__ void finish_row(const NormArgs& a, long long row, const int (&n)[CH], const int (&e0)[CH], const Raw8<T> (&xr)[CH],
-                                           const Raw8<R> (&rr)[CH], const Vector8<T> (&gr)[EARLY ? CH : 1], float (*s_sum)[32], int warps,
+                                           const Raw8<R> (&rr)[CH], const Vector8<T> (&gr)[EARLY ? CH : 1], float* sums, int slots, int warps,
                                            int warp0, int lane) {
   float v[CH][8];
 #pragma unroll
   for (int c = 0; c < CH; ++c) unpack8<T>(xr[c], v[c]);
   if (POST && a.post)
-    normalise<T, VEC, CH, EARLY>(v, n, e0, a, a.w_post, a.b_post, a.w_post_f32, a.b_post_f32, s_sum[0], s_sum[1], warps, warp0, lane);
+    normalise<T, VEC, CH, EARLY, LAYER>(v, n, e0, a, a.w_post, a.b_post, a.w_post_f32, a.b_post_f32, sums, slots, warps, warp0, lane);
 
   float scale = a.scale;
   if (a.gate_mode == B200MOE_GATE_TOKEN && row < a.M)
@@ -161,7 +201,7 @@ __device__ __forceinline__ void finish_row(const NormArgs& a, long long row, con
     if (a.hidden != nullptr) store8<R, VEC>(static_cast<R*>(a.hidden) + row * a.ldh + e0[c], n[c], v[c]);
   }
   if (!PRE || !a.pre) return;
-  normalise<T, VEC, CH, EARLY>(v, n, e0, a, a.w_pre, a.b_pre, a.w_pre_f32, a.b_pre_f32, s_sum[2], s_sum[3], warps, warp0, lane);
+  normalise<T, VEC, CH, EARLY, LAYER>(v, n, e0, a, a.w_pre, a.b_pre, a.w_pre_f32, a.b_pre_f32, sums + kNormSums * slots, slots, warps, warp0, lane);
   if (a.y_scale == nullptr) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) store8<T, VEC>(static_cast<T*>(a.y) + row * a.H + e0[c], n[c], v[c]);
@@ -173,10 +213,10 @@ __device__ __forceinline__ void finish_row(const NormArgs& a, long long row, con
 }
 
 // POST, PRE: norms that the call may have
-template <typename T, typename R, bool VEC, int CH, int THREADS, bool POST, bool PRE>
-__global__ void __launch_bounds__(THREADS)
+template <typename T, typename R, bool VEC, int CH, int THREADS, bool LAYER, bool POST, bool PRE>
+__global__ void __launch_bounds__(THREADS, THREADS == 512 && CH == 1 ? 3 : 0)
 block_norm_kernel(const NormArgs a) {
-  __shared__ float s_sum[kMaxSums][32];
+  __shared__ float s_sum[2 * kNormSums * 32];
   griddep_wait();
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31;
@@ -197,7 +237,7 @@ block_norm_kernel(const NormArgs a) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) load_gate_chunk<T, VEC>(a, row, n[c], e0[c], gr[c]);
   }
-  finish_row<T, R, VEC, CH, true, POST, PRE>(a, row, n, e0, xr, rr, gr, s_sum, warps, warp0, lane);
+  finish_row<T, R, VEC, CH, true, LAYER, POST, PRE>(a, row, n, e0, xr, rr, gr, s_sum, 32, warps, warp0, lane);
 }
 
 __device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
@@ -212,12 +252,12 @@ __device__ __forceinline__ void copies_wait() {
 // Many rows: every thread keeps its elements of the next S - 1 rows on their way into shared memory while the CTA works on one, so
 // that memory stays busy through the sums' round trips however few CTAs fit.  Weights, biases and a gate per channel are copied once and
 // stay there (from L2 each of them cost a row another round trip).  A thread reads only what it has copied itself.
-template <typename T, typename R, int CH, int S>
+template <typename T, typename R, int CH, int S, bool LAYER>
 __global__ void __launch_bounds__(512, 1)
 block_norm_ring_kernel(const NormArgs args, int stage_bytes) {
   NormArgs a = args;
   extern __shared__ __align__(16) uint8_t ring[];
-  __shared__ float s_sum[2][kMaxSums][32];
+  __shared__ float s_sum[2][2 * kNormSums * 16];
   griddep_wait();
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31, warps = a.team >> 5;
@@ -281,7 +321,7 @@ block_norm_ring_kernel(const NormArgs args, int stage_bytes) {
       load8<T, true>(reinterpret_cast<const T*>(at) + e0[c], n[c], xr[c]);
       if (a.residual != nullptr) load8<R, true>(reinterpret_cast<const R*>(at + r_at) + e0[c], n[c], rr[c]);
     }
-    finish_row<T, R, true, CH, false>(a, row, n, e0, xr, rr, gr, s_sum[turn], warps, 0, lane);
+    finish_row<T, R, true, CH, false, LAYER>(a, row, n, e0, xr, rr, gr, s_sum[turn], 16, warps, 0, lane);
     turn ^= 1;
     if (++s == S) s = 0;
   }
@@ -295,7 +335,7 @@ __global__ void __launch_bounds__(512, 2)
 block_norm_stream_kernel(const NormArgs a, int stages, int stage_bytes) {
   constexpr int CH = 2;
   extern __shared__ __align__(16) uint8_t ring[];
-  __shared__ float s_sum[2][kMaxSums][32];
+  __shared__ float s_sum[2][2 * kNormSums * 16];
   griddep_wait();
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31, warps = a.team >> 5;
@@ -338,11 +378,10 @@ block_norm_stream_kernel(const NormArgs a, int stages, int stage_bytes) {
   for (int s = 0; s < stages - 1; ++s) fetch(s * stage_bytes);
 
   const bool channel = a.gate_mode == B200MOE_GATE_CHANNEL;
-  auto sum = [&](float v, float* slots) { return team_sum(v, slots, warps, 0, lane); };
-  const float per = 1.f / static_cast<float>(a.H);
+  const float per = 1.f / static_cast<float>(a.H);      // (rounded: the mean is corrected, and nothing else sees more than 2^-24 of it)
   // v = (v - mean) * rsqrt(var + eps) * (offset + w) + b.  The vectors stay in L1.
   const unsigned long long offset2 = pack_f32x2(a.offset, a.offset);
-  auto normalise2 = [&](unsigned long long (&v)[CH][4], const void* w, bool w_f32, const void* b, bool b_f32, float* s0, float* s1) {
+  auto normalise2 = [&](unsigned long long (&v)[CH][4], const void* w, bool w_f32, const void* b, bool b_f32, float* sums) {
     constexpr bool EARLY = FAST && FORM != kBetween;      // (two norms: the registers for it are not there, 30.2 us became 33.5)
     Raw8<T> early[EARLY ? CH : 1];
     if (EARLY && w != nullptr) {
@@ -357,7 +396,7 @@ block_norm_stream_kernel(const NormArgs a, int stages, int stage_bytes) {
         for (int i = 0; i < 4; ++i) t = add2(t, v[c][i]);
       float lo, hi;
       unpack_f32x2(t, lo, hi);
-      const float mean = sum(lo + hi, s0) * per;
+      const float mean = team_sum(lo + hi, sums, warps, 0, lane) * per;
       const unsigned long long m2 = pack_f32x2(-mean, -mean);
 #pragma unroll
       for (int c = 0; c < CH; ++c)
@@ -371,7 +410,24 @@ block_norm_stream_kernel(const NormArgs a, int stages, int stage_bytes) {
       for (int i = 0; i < 4; ++i) t = fma2(v[c][i], v[c][i], t);
     float lo, hi;
     unpack_f32x2(t, lo, hi);
-    const float r = rsqrtf(sum(lo + hi, s1) * per + a.eps);
+    float r, shift = 0.f;
+    if (LAYER) {
+      unsigned long long t1 = 0;
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t1 = add2(t1, v[c][i]);
+      float q = lo + hi, d;
+      unpack_f32x2(t1, lo, hi);
+      d = lo + hi;
+      team_sum(d, q, sums + 16, 16, warps, 0, lane);
+      d *= per;
+      r = rsqrtf(variance(q * per, d) + a.eps);
+      shift = -d * r;
+    } else {
+      r = rsqrtf(team_sum(lo + hi, sums, warps, 0, lane) * per + a.eps);
+    }
+    const unsigned long long shift2 = pack_f32x2(shift, shift);
     const unsigned long long r2 = pack_f32x2(r, r);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -387,10 +443,10 @@ block_norm_stream_kernel(const NormArgs a, int stages, int stage_bytes) {
           unpack_vector<T>(wr, w_f32, f);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[c][i] = mul2(mul2(v[c][i], r2), add2(pack_f32x2(f[2 * i], f[2 * i + 1]), offset2));
+        for (int i = 0; i < 4; ++i) v[c][i] = mul2(LAYER ? fma2(v[c][i], r2, shift2) : mul2(v[c][i], r2), add2(pack_f32x2(f[2 * i], f[2 * i + 1]), offset2));
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[c][i] = mul2(v[c][i], r2);
+        for (int i = 0; i < 4; ++i) v[c][i] = LAYER ? fma2(v[c][i], r2, shift2) : mul2(v[c][i], r2);
       }
       if (b != nullptr) {
         Vector8<T> br;
@@ -443,7 +499,7 @@ block_norm_stream_kernel(const NormArgs a, int stages, int stage_bytes) {
       load8<T, true>(reinterpret_cast<const T*>(at) + e0[c], 8, x);
       unpack4x2<T>(x, v[c]);
     }
-    if (FORM != kBefore) normalise2(v, a.w_post, a.w_post_f32, a.b_post, a.b_post_f32, s_sum[turn][0], s_sum[turn][1]);
+    if (FORM != kBefore) normalise2(v, a.w_post, a.w_post_f32, a.b_post, a.b_post_f32, s_sum[turn]);
     const unsigned long long s2 = pack_f32x2(scale, scale);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -475,7 +531,7 @@ block_norm_stream_kernel(const NormArgs a, int stages, int stage_bytes) {
     }
     ph += step_h;
     if (FORM != kAfter) {
-      normalise2(v, a.w_pre, a.w_pre_f32, a.b_pre, a.b_pre_f32, s_sum[turn][2], s_sum[turn][3]);
+      normalise2(v, a.w_pre, a.w_pre_f32, a.b_pre, a.b_pre_f32, s_sum[turn] + kNormSums * 16);
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         float y[8];
@@ -512,7 +568,7 @@ cudaError_t launch_stream(const NormArgs& a, int ctas, int stages, int stage_byt
 
 template <typename T, typename R, int CH, int S>
 cudaError_t launch_ring(const NormArgs& a, int ctas, int stage_bytes, int kept_bytes, int num_sms, cudaStream_t stream) {
-  auto kernel = block_norm_ring_kernel<T, R, CH, S>;
+  auto kernel = a.layer ? block_norm_ring_kernel<T, R, CH, S, true> : block_norm_ring_kernel<T, R, CH, S, false>;
   const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
   if (err != cudaSuccess) return err;
   const int grid = static_cast<int>(std::min<long long>(a.M, static_cast<long long>(ctas) * num_sms));
@@ -563,11 +619,20 @@ int launch_rows(NormArgs a, int num_sms, cudaStream_t stream) {
   a.rows_per_cta = a.M > 2 * num_sms && a.team < 128 ? 128 / a.team : 1;
   const dim3 grid((a.M + a.rows_per_cta - 1) / a.rows_per_cta), block(a.team * a.rows_per_cta);
   note_launch("block_norm_kernel");
-  auto kernel = ch == 4    ? block_norm_kernel<T, R, VEC, 4, 512, true, true>
-                : ch == 2  ? block_norm_kernel<T, R, true, 2, 512, true, true>      // (rows of up to 512, too narrow to stream)
-                : !a.post  ? block_norm_kernel<T, R, VEC, 1, 1024, false, true>
-                : !a.pre   ? block_norm_kernel<T, R, VEC, 1, 1024, true, false>
-                           : block_norm_kernel<T, R, VEC, 1, 1024, true, true>;
+  // A layer norm before a block needs a few registers more than the RMS norm; with 40 four of its CTAs of 352 threads share an SM, and three with
+  // more (1001 x 2600, fp16: 7.3 us and 9.1).  Rows of 16-bit types fit into 40 without spills.
+  constexpr bool SLIM = VEC && sizeof(T) == 2 && sizeof(R) == 2;
+  const bool slim = SLIM && block.x <= 512;
+  auto pick = [&](auto layer) {
+    constexpr bool L = decltype(layer)::value;
+    return ch == 4   ? block_norm_kernel<T, R, VEC, 4, 512, L, true, true>
+           : ch == 2 ? block_norm_kernel<T, R, true, 2, 512, L, true, true>      // (rows of up to 512, too narrow to stream)
+           : !a.post ? (L && slim ? block_norm_kernel<T, R, VEC, 1, SLIM && L ? 512 : 1024, L, false, true>
+                                  : block_norm_kernel<T, R, VEC, 1, 1024, L, false, true>)
+           : !a.pre  ? block_norm_kernel<T, R, VEC, 1, 1024, L, true, false>
+                     : block_norm_kernel<T, R, VEC, 1, 1024, L, true, true>;
+  };
+  auto kernel = a.layer ? pick(std::true_type{}) : pick(std::false_type{});
   err = launch_kernel(kernel, grid, block, 0, stream, a.pdl != 0, a);
   return err == cudaSuccess ? B200MOE_OK : B200MOE_ERR_CUDA;
 }
