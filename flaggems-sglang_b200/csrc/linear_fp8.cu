@@ -38,7 +38,7 @@ __device__ __forceinline__ float bias_at(const LinearArgs& a, int n) {
 constexpr int kQuantRuns = 4;
 template <typename T>
 __global__ void __launch_bounds__(256)
-linear_quant_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q, float* __restrict__ scales, int K, int G) {
+linear_quant_kernel(const T* x, long long ldx, uint8_t* q, float* scales, int K, int G) {
   griddep_wait();
   griddep_launch_dependents();
   const int halves = blockDim.x >> 4, g0 = blockIdx.y * halves * kQuantRuns + (threadIdx.x >> 4), l16 = threadIdx.x & 15;
@@ -759,10 +759,11 @@ fp8_linear_token_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_c
           ws[b] = a.w_scale + (lw[b] ? static_cast<size_t>(n * BLOCKS + b) * a.G : 0);
         }
         for (int kb = kb0; kb < kb1; ++kb, ++k) {
-          const float v0 = l0 ? __ldg(x0 + kb) : 0.f, v1 = l1 ? __ldg(x1 + kb) : 0.f;
+          // (no read-only loads: the kernel before may still write the scales when this one starts)
+          const float v0 = l0 ? x0[kb] : 0.f, v1 = l1 ? x1[kb] : 0.f;
           float w[BLOCKS];
 #pragma unroll
-          for (int b = 0; b < BLOCKS; ++b) w[b] = lw[b] ? __ldg(ws[b] + kb) : 0.f;
+          for (int b = 0; b < BLOCKS; ++b) w[b] = lw[b] ? ws[b][kb] : 0.f;
           if (k >= 2) {
             const long long p = k - 2;
             if (!(ok = mbar_wait(smem_u32(&bar_pfull[p % NBUF]), static_cast<uint32_t>(p / NBUF) & 1, abort_flag, DEV_TIMEOUT_EPILOGUE))) break;
