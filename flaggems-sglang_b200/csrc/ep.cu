@@ -185,7 +185,7 @@ ep_dispatch_kernel(const EpDispatchArgs a) {
     } else {
       const uint4* src = reinterpret_cast<const uint4*>(xrow);
       for (int c = threadIdx.x; c < a.H / 8; c += blockDim.x) {
-        const uint4 v = __ldg(src + c);
+        const uint4 v = __ldcg(src + c);
         for (int d = 0; d < a.world; ++d)
           if (dest_mask & (1u << d))
             reinterpret_cast<uint4*>(a.heap[d] + a.L.recv_x + row * a.L.x_row_bytes)[c] = v;

@@ -9,7 +9,7 @@ namespace {
 
 template <int MODE, typename T>
 __global__ void __launch_bounds__(256)
-moe_gemm_simt_kernel(const T* __restrict__ w, const T* __restrict__ x, const GemmArgs a) {
+moe_gemm_simt_kernel(const T* w, const T* x, const GemmArgs a) {
   const int rows = a.meta[1];
   const int r = blockIdx.x;
   if (r >= rows) return;

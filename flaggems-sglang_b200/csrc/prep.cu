@@ -20,9 +20,9 @@ namespace {
 constexpr int kGatherSeg = 128;      // 16-byte chunks per warp and step
 
 __global__ void __launch_bounds__(256)
-gather_rows_kernel(const uint4* __restrict__ x, uint4* __restrict__ xs, const int* __restrict__ sorted_ids,
-                   const int* __restrict__ meta, int P, int topk, int chunks_per_row, int cap,
-                   uint4* __restrict__ zero, long long zero_chunks, const float* __restrict__ sc_src,
+gather_rows_kernel(const uint4* x, uint4* __restrict__ xs, const int* sorted_ids,
+                   const int* meta, int P, int topk, int chunks_per_row, int cap,
+                   uint4* __restrict__ zero, long long zero_chunks, const float* sc_src,
                    float* __restrict__ sc_dst, int G, int ld, const FlagWait fw) {
   griddep_wait();
   griddep_launch_dependents();
@@ -39,7 +39,7 @@ gather_rows_kernel(const uint4* __restrict__ x, uint4* __restrict__ xs, const in
       if (r >= rows) continue;
       const int slot = sorted_ids[r];
       if (slot >= 0 && slot < P)
-        sc_dst[static_cast<size_t>(g) * ld + r] = __ldg(sc_src + static_cast<size_t>(slot / topk) * G + g);
+        sc_dst[static_cast<size_t>(g) * ld + r] = __ldcg(sc_src + static_cast<size_t>(slot / topk) * G + g);
     }
   }
   const int lane = thread & 31;
@@ -55,7 +55,7 @@ gather_rows_kernel(const uint4* __restrict__ x, uint4* __restrict__ xs, const in
     uint4 v[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-      if (c0 + 32 * q < chunks_per_row) v[q] = __ldg(src + c0 + 32 * q);
+      if (c0 + 32 * q < chunks_per_row) v[q] = __ldcg(src + c0 + 32 * q);
 #pragma unroll
     for (int q = 0; q < 4; ++q)
       if (c0 + 32 * q < chunks_per_row) dst[c0 + 32 * q] = v[q];
@@ -82,7 +82,7 @@ __device__ __forceinline__ int routed_row(const RouteSource& route, const RowTab
 }
 
 __global__ void __launch_bounds__(256)
-gather_routed_kernel(const uint4* __restrict__ x, uint4* __restrict__ xs, const RouteSource route, int P, int E, int BT, int topk,
+gather_routed_kernel(const uint4* x, uint4* __restrict__ xs, const RouteSource route, int P, int E, int BT, int topk,
                      int chunks_per_row, uint4* __restrict__ zero, long long zero_chunks) {
   extern __shared__ __align__(16) uint8_t route_smem[];
   const RowTables t = row_tables(route_smem, E);
@@ -102,7 +102,7 @@ gather_routed_kernel(const uint4* __restrict__ x, uint4* __restrict__ xs, const 
     const uint4* src = x + static_cast<size_t>(slot / topk) * chunks_per_row;
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-      if (c0 + 32 * q < chunks_per_row) v[q] = __ldg(src + c0 + 32 * q);
+      if (c0 + 32 * q < chunks_per_row) v[q] = __ldcg(src + c0 + 32 * q);
   };
   const int units = P * segs;
   int u = thread >> 5;
@@ -161,8 +161,8 @@ __device__ __forceinline__ uint32_t quantise_group(const float (&v)[4], int lane
 // scale_t != 0: scales stored [K/128][ld_scale] (group-major) instead of [rows][K/128].
 template <typename T>
 __global__ void __launch_bounds__(256)
-group_quant_fp8_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scales,
-                       const int* __restrict__ sorted_ids, const int* __restrict__ meta, int P, int topk,
+group_quant_fp8_kernel(const T* x, uint8_t* __restrict__ q, float* __restrict__ scales,
+                       const int* sorted_ids, const int* meta, int P, int topk,
                        int n_rows_static, int K, int scale_t, int ld_scale, uint4* __restrict__ zero,
                        long long zero_chunks) {
   griddep_wait();
@@ -216,8 +216,8 @@ group_quant_fp8_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* 
 constexpr int kQuantRun = 8;      // groups of a run at most; few tokens are dealt out in shorter ones
 template <typename T>
 __global__ void __launch_bounds__(256)
-group_quant_slots_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scales, const RouteSource route,
-                         const int* __restrict__ slot_row, int P, int E, int BT, int topk, int M, int K, int run, int ld_scale,
+group_quant_slots_kernel(const T* x, uint8_t* __restrict__ q, float* __restrict__ scales, const RouteSource route,
+                         const int* slot_row, int P, int E, int BT, int topk, int M, int K, int run, int ld_scale,
                          uint4* __restrict__ zero, long long zero_chunks) {
   extern __shared__ __align__(16) uint8_t route_smem[];
   __shared__ __align__(16) uint2 s_x[8][kQuantRun][32];
@@ -274,7 +274,7 @@ group_quant_slots_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float
 
 template <typename T>
 __global__ void __launch_bounds__(256)
-finalize_kernel(const float4* __restrict__ acc, T* __restrict__ out, size_t n4, float scale, const FlagWait fw) {
+finalize_kernel(const float4* acc, T* __restrict__ out, size_t n4, float scale, const FlagWait fw) {
   griddep_wait();
   griddep_launch_dependents();
   wait_for_peers(fw);
@@ -290,7 +290,7 @@ finalize_kernel(const float4* __restrict__ acc, T* __restrict__ out, size_t n4, 
 // One thread per (token, run of 8 columns): fp32 sum of the token's valid pair rows.
 template <typename T>
 __global__ void __launch_bounds__(256)
-finalize_pairs_kernel(const uint4* __restrict__ pairs, const uint8_t* __restrict__ pair_valid, uint4* __restrict__ out,
+finalize_pairs_kernel(const uint4* pairs, const uint8_t* pair_valid, uint4* __restrict__ out,
                       int M, int topk, int chunks_per_row, float scale, const FlagWait fw) {
   griddep_wait();
   griddep_launch_dependents();
@@ -314,7 +314,7 @@ finalize_pairs_kernel(const uint4* __restrict__ pairs, const uint8_t* __restrict
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const size_t slot = static_cast<size_t>(t) * topk + j0 + u;
-        v[u] = ok[u] ? __ldg(pairs + slot * chunks_per_row + c) : make_uint4(0, 0, 0, 0);
+        v[u] = ok[u] ? __ldcg(pairs + slot * chunks_per_row + c) : make_uint4(0, 0, 0, 0);
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {

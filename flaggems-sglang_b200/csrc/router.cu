@@ -46,7 +46,7 @@ __device__ __forceinline__ void warp_argmax(float& v, int& idx) {
 
 template <typename TL>
 __global__ void __launch_bounds__(kRouterWarps * 32)
-route_topk_kernel(const TL* __restrict__ logits, const float* __restrict__ bias, int M, int E, int topk,
+route_topk_kernel(const TL* logits, const float* bias, int M, int E, int topk,
                   int scoring, int renorm, int n_group, int topk_group, float scale,
                   float* __restrict__ out_w, int* __restrict__ out_ids) {
   extern __shared__ float rsm[];

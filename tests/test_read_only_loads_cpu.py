@@ -36,5 +36,16 @@ def test_operators_around_the_experts(name):
         assert not re.search(r"const\s+\w+\s*\*\s*__restrict__", arguments), kernel
 
 
+@pytest.mark.parametrize("name", ["prep.cu", "router.cu", "ep.cu", "gemm_simt.cu"])
+def test_rows_that_enter_the_experts(name):
+    """Tokens come from a norm that lets the next kernel start early, router logits from a product that does; lists, sorted rows and pairs from the
+    kernels of the call itself."""
+    text = _code(name)
+    assert "__ldg(" not in text and "ld.global.nc" not in text
+    for kernel, arguments in _kernel_arguments(text):
+        assert not re.search(r"const\s+\w+\s*\*\s*__restrict__", arguments), kernel
+
+
 def test_the_kernels_are_found():
     assert {k for k, _ in _kernel_arguments(_code("linear_fp8.cu"))} >= {"linear_quant_kernel", "fp8_linear_decode_kernel", "fp8_linear_token_kernel"}
+    assert {k for k, _ in _kernel_arguments(_code("prep.cu"))} >= {"gather_rows_kernel", "gather_routed_kernel", "group_quant_fp8_kernel", "finalize_pairs_kernel"}
