@@ -1432,6 +1432,27 @@ int b200moe_fp8_linear(const b200moe_linear* p, const void* x, const float* x_sc
   return launch_fp8_linear(a, sms, static_cast<cudaStream_t>(stream));
 }
 
+int b200moe_status_alloc(int32_t** status) {
+  if (status == nullptr) return B200MOE_ERR_BAD_ARG;
+  *status = nullptr;
+  // (relaxed: what another stream captures does not forbid this thread to allocate or to wait for a stream of its own)
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return B200MOE_ERR_CUDA;
+  void* word = nullptr;
+  cudaStream_t stream = nullptr;
+  cudaError_t err = cudaMalloc(&word, 256);
+  if (err == cudaSuccess) err = cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking);
+  if (err == cudaSuccess) err = cudaMemsetAsync(word, 0, 256, stream);
+  if (err == cudaSuccess) err = cudaStreamSynchronize(stream);
+  if (stream != nullptr) (void)cudaStreamDestroy(stream);
+  if (err != cudaSuccess && word != nullptr) (void)cudaFree(word);
+  if (err != cudaSuccess) (void)cudaGetLastError();
+  (void)cudaThreadExchangeStreamCaptureMode(&mode);
+  if (err != cudaSuccess) return B200MOE_ERR_CUDA;
+  *status = static_cast<int32_t*>(word);
+  return B200MOE_OK;
+}
+
 int b200moe_debug_resident_cta_pairs(void) { return gemm_tc2_resident_pairs(); }
 
 int b200moe_launch_stats(long long* total_launches, char* last_call_names, size_t names_bytes) {

@@ -123,6 +123,7 @@ SYMBOLS = {
     "b200moe_selftest_timeout": (C.c_int, [C.c_uint64, C.c_void_p, C.c_void_p, C.c_void_p]),
     "b200moe_per_token_group_quant_fp8": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p,
                                                     C.c_void_p, C.c_void_p]),
+    "b200moe_status_alloc": (C.c_int, [C.c_void_p]),
     "b200moe_block_norm": (C.c_int, [C.c_void_p] * 12),
     "b200moe_gated_activation": (C.c_int, [C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, C.c_float,
                                            C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),

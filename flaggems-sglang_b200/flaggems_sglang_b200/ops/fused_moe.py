@@ -80,11 +80,27 @@ def release_workspaces(device=None) -> None:
         _workspaces.pop(key)
 
 
+class _DeviceWord:
+    """One int32 at a device address, as torch takes it over."""
+
+    def __init__(self, address: int):
+        self.__cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (address, False), "strides": None, "version": 3}
+
+
 def _status_word(dev: torch.device) -> torch.Tensor:
+    """The word that kernels on this device report time-outs into.  It comes from the library, not from torch: a call within a capture would get
+    memory of that graph, which every replay clears, and which holds anything until the first."""
     st = _status.get(dev.index)
     if st is None:
-        st = torch.zeros(1, dtype=torch.int32, device=dev)
-        _status[dev.index] = st
+        word = C.c_void_p()
+        with torch.cuda.device(dev):
+            rc = _lib.lib().b200moe_status_alloc(C.byref(word))
+            if rc != _lib.OK and not _capturing():
+                torch.cuda.empty_cache()            # (torch may hold all of the memory)
+                rc = _lib.lib().b200moe_status_alloc(C.byref(word))
+            if rc != _lib.OK:
+                _lib.check(rc, "status_alloc")
+            st = _status.setdefault(dev.index, torch.as_tensor(_DeviceWord(word.value), device=dev))
     return st
 
 

@@ -464,6 +464,13 @@ int b200moe_debug_resident_cta_pairs(void);
  */
 int b200moe_selftest_timeout(uint64_t limit_ns, int32_t *status, int32_t *observed, void *stream);
 
+/*
+ * A status word for the calls above on the current device: device int32, zero when this returns, there as long as the
+ * process.  It may be asked for while a stream is being captured into a graph and belongs to no graph then (a word from the
+ * capture's own memory would be cleared by every replay, with what other calls had reported).
+ */
+int b200moe_status_alloc(int32_t **status);
+
 #ifdef __cplusplus
 }
 #endif
