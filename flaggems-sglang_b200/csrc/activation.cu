@@ -146,8 +146,7 @@ template <typename T, int ACT>
 int launch_typed(const ActArgs& a, cudaStream_t stream) {
   const int chunks = (a.I + 7) / 8;
   const int threads = std::min(256, ((chunks + kRuns - 1) / kRuns + 31) / 32 * 32), per_cta = threads * kRuns;
-  const int segments = (chunks + per_cta - 1) / per_cta;
-  if (segments > 65535) return B200MOE_ERR_TOO_LARGE;
+  const int segments = (chunks + per_cta - 1) / per_cta;      // (B200MOE_ACT_MAX_I: at most 65535)
   note_launch("gated_activation_kernel");
   const dim3 grid(a.M, segments);
   cudaError_t err = a.vec ? launch_kernel(gated_activation_kernel<T, ACT, true>, grid, dim3(threads), 0, stream, a.pdl != 0, a)

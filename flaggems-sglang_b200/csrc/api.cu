@@ -1329,7 +1329,7 @@ int b200moe_block_norm(const b200moe_norm* p, const void* x, const void* residua
                        void* stream) {
   if (p == nullptr || p->struct_bytes != static_cast<int32_t>(sizeof(b200moe_norm))) return B200MOE_ERR_BAD_ARG;
   if (p->M < 0 || p->H <= 0 || (!p->post && !p->pre)) return B200MOE_ERR_BAD_ARG;
-  if (p->H > B200MOE_NORM_MAX_H || p->M > (1 << 30)) return B200MOE_ERR_TOO_LARGE;
+  if (p->H > B200MOE_NORM_MAX_H || p->M > B200MOE_NORM_MAX_ROWS) return B200MOE_ERR_TOO_LARGE;
   if (p->dtype < B200MOE_DTYPE_BF16 || p->dtype > B200MOE_DTYPE_FP32) return B200MOE_ERR_BAD_ARG;
   if (p->kind != B200MOE_NORM_RMS && p->kind != B200MOE_NORM_LAYER) return B200MOE_ERR_BAD_ARG;
   if (p->gate_mode < B200MOE_GATE_NONE || p->gate_mode > B200MOE_GATE_FULL) return B200MOE_ERR_BAD_ARG;
@@ -1376,7 +1376,7 @@ int b200moe_gated_activation(const void* x, int64_t ldx, int dtype, int M, int I
   if (M < 0 || I <= 0 || dtype < B200MOE_DTYPE_BF16 || dtype > B200MOE_DTYPE_FP32 || activation < B200MOE_ACT_SILU ||
       activation > B200MOE_ACT_SWIGLU_OAI)
     return B200MOE_ERR_BAD_ARG;
-  if (I > (1 << 29)) return B200MOE_ERR_TOO_LARGE;
+  if (I > B200MOE_ACT_MAX_I || M > B200MOE_MAX_ROWS) return B200MOE_ERR_TOO_LARGE;
   if (M == 0) return B200MOE_OK;
   if (x == nullptr || y == nullptr || ldx < 2 * static_cast<int64_t>(I)) return B200MOE_ERR_BAD_ARG;
   ActArgs a = {};
@@ -1394,7 +1394,7 @@ static int linear_args(const b200moe_linear* p, LinearArgs* a) {
   if (p->out_dtype < B200MOE_DTYPE_BF16 || p->out_dtype > B200MOE_DTYPE_FP32) return B200MOE_ERR_BAD_ARG;
   if (p->bias_dtype < B200MOE_DTYPE_BF16 || p->bias_dtype > B200MOE_DTYPE_FP32) return B200MOE_ERR_BAD_ARG;
   if (p->K % 16 != 0) return B200MOE_ERR_UNSUPPORTED;
-  if (p->K > B200MOE_LINEAR_MAX_K) return B200MOE_ERR_TOO_LARGE;
+  if (p->K > B200MOE_LINEAR_MAX_K || p->M > B200MOE_MAX_ROWS || p->N > B200MOE_MAX_ROWS) return B200MOE_ERR_TOO_LARGE;
   *a = {};
   a->M = p->M; a->N = p->N; a->K = p->K; a->G = (p->K + 127) / 128;
   a->ldx = p->ldx; a->ldw = p->ldw; a->x_dtype = p->x_dtype; a->out_dtype = p->out_dtype; a->bias_dtype = p->bias_dtype;

@@ -127,7 +127,7 @@ PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Tensor& t = *x.t;
   const int64_t h = t.size(-1), m = t.numel() / h;
   const int dt = code_of(t.scalar_type());
-  if (dt < 0 || h > B200MOE_NORM_MAX_H || m > (1 << 30)) return none();
+  if (dt < 0 || h > B200MOE_NORM_MAX_H || m > B200MOE_NORM_MAX_ROWS) return none();
   if (residual.t != nullptr && (!residual.on(t) || residual.t->sizes() != t.sizes() ||
                                 (residual.t->scalar_type() != t.scalar_type() && residual.t->scalar_type() != at::kFloat)))
     return none();
@@ -200,7 +200,7 @@ PyObject* activation(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Tensor& t = *x.t;
   const int64_t w = t.size(-1), m = t.numel() / w, i = w / 2;
   const int dt = code_of(t.scalar_type());
-  if (dt < 0 || w % 2 != 0 || m > 0x7fffffff || i > (1 << 29)) return none();
+  if (dt < 0 || w % 2 != 0 || m > B200MOE_MAX_ROWS || i > B200MOE_ACT_MAX_I) return none();
   const int kind = static_cast<int>(PyLong_AsLong(args[0]));
   at::Tensor y, scale;
   int rc;
@@ -227,7 +227,7 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Tensor &t = *x.t, &w = *weight.t, &ws = *weight_scale.t;
   if (w.dim() != 2 || w.scalar_type() != kFp8 || w.device() != t.device() || w.size(0) <= 0 || w.size(1) != t.size(-1)) return none();
   const int64_t rows = w.size(0), k = w.size(1), m = t.numel() / k, g = (k + 127) / 128;
-  if (k % 16 != 0 || k > B200MOE_LINEAR_MAX_K || rows > 0x7fffffff || m > 0x7fffffff) return none();
+  if (k % 16 != 0 || k > B200MOE_LINEAR_MAX_K || rows > B200MOE_MAX_ROWS || m > B200MOE_MAX_ROWS) return none();
   if (w.stride(1) != 1 || (rows > 1 && (w.stride(0) < k || w.stride(0) % 16 != 0))) return none();
   if (!weight_scale.on(t) || ws.scalar_type() != at::kFloat || ws.dim() != 2 || ws.size(0) != (rows + 127) / 128 || ws.size(1) != g) return none();
   const bool fp8 = t.scalar_type() == kFp8;

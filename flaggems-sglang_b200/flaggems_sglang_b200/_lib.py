@@ -60,6 +60,9 @@ GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_FULL = 0, 1, 2, 3
 NORM_RMS, NORM_LAYER = 0, 1
 NORM_MAX_H = 16384
 LINEAR_MAX_K = 65536
+ACT_MAX_I = 65535 * 4096
+MAX_ROWS = 0x7fffff00
+NORM_MAX_ROWS = 1 << 30
 X_E4M3 = -1
 
 

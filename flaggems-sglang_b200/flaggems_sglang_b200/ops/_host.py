@@ -57,6 +57,17 @@ def strides_of(shape) -> tuple:
     return tuple(reversed(out))
 
 
+def counted(m: int, most: int) -> int:
+    """``m`` rows (or elements of a row): a description holds 32 bits, which a larger number would not fit into."""
+    if m > most:
+        raise ValueError(f"sizes of more than {most} are not supported")
+    return m
+
+
+def rows_of(t: torch.Tensor, h: int, most: int) -> int:
+    return counted(t.numel() // h, most)
+
+
 def as_rows(t: torch.Tensor, h: int) -> torch.Tensor:
     """[rows, h] with contiguous rows: a view where the strides allow it, else a copy."""
     t = t if t.dim() == 2 else t.reshape(-1, h)

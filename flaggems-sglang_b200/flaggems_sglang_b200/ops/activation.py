@@ -21,7 +21,8 @@ def _make_plan(x, activation, quantize):
         raise ValueError(f"Unsupported activation: {activation}")
     assert x.dtype in _host.DTYPES, "x must be bfloat16, float16 or float32"
     assert x.dim() >= 1 and x.shape[-1] > 0 and x.shape[-1] % 2 == 0, "x must be [..., 2I]"
-    i = x.shape[-1] // 2
+    i = _host.counted(x.shape[-1] // 2, _lib.ACT_MAX_I)
+    _host.rows_of(x, 2 * i, _lib.MAX_ROWS)
     x2 = _host.as_rows(x, 2 * i)
     lead = tuple(x.shape[:-1])
     y, groups = lead + (i,), lead + (-(-i // 128),)

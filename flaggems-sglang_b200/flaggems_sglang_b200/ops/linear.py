@@ -36,6 +36,8 @@ def _make_plan(x, weight, weight_scale, bias, x_scale, out_dtype, tile, split, f
     dev = x.device
     assert x.dim() >= 1 and x.shape[-1] == k, "x and weight differ in K"
     assert n > 0 and k > 0 and k % 16 == 0, "K must be a multiple of 16"
+    _host.counted(n, _lib.MAX_ROWS)
+    _host.rows_of(x, _host.counted(k, _lib.LINEAR_MAX_K), _lib.MAX_ROWS)
     g = -(-k // 128)
     assert weight.device == dev and weight_scale.device == dev, "x, weight and weight_scale must be on one device"
     assert weight_scale.shape == (-(-n // 128), g), "weight_scale must be [ceil(N/128), ceil(K/128)]"

@@ -68,6 +68,7 @@ def _make_plan(x, post, pre, w_post, b_post, w_pre, b_pre, residual, gate, resid
     h = x.shape[-1]
     if h > _lib.NORM_MAX_H:
         raise ValueError(f"rows of more than {_lib.NORM_MAX_H} elements are not supported")
+    _host.rows_of(x, h, _lib.NORM_MAX_ROWS)
     if residual is not None:
         assert residual.shape == x.shape and residual.device == x.device, "residual must have x's shape and device"
         assert residual.dtype in (x.dtype, torch.float32), "residual must have x's type or float32"

@@ -351,7 +351,8 @@ int b200moe_per_token_group_quant_fp8(const void *x, int dtype, int rows, int K,
 
 /*
  * Operators around the experts.  All launch asynchronously, allocate nothing and never synchronise; row strides are in
- * elements and at least the row's length; empty batches (M = 0) return at once.
+ * elements and at least the row's length; empty batches (M = 0) return at once.  M (and N) up to B200MOE_MAX_ROWS,
+ * for the norms up to B200MOE_NORM_MAX_ROWS.
  *
  * Norms before and after a block with its gate, residual scale and residual add (the reference's Gemma RMSNorm operators,
  * src/flaggems_sglang/ops/gemma_rms_norm.py:18-117, are the RMS form with weight_offset 1):
@@ -361,6 +362,8 @@ int b200moe_per_token_group_quant_fp8(const void *x, int dtype, int rows, int K,
  *   norm(v) = (v - mean) * rsqrt(mean((v - mean)^2) + eps) * (weight_offset + w) + b;  B200MOE_NORM_RMS: mean = 0
  * in fp32, h and y each rounded once.  A null weight counts as weight_offset + w = 1, a null bias as 0.
  */
+#define B200MOE_MAX_ROWS 0x7fffff00 /* whole tiles of 256 below 2^31 */
+#define B200MOE_NORM_MAX_ROWS (1 << 30)
 #define B200MOE_NORM_RMS 0
 #define B200MOE_NORM_LAYER 1
 #define B200MOE_GATE_NONE 0
@@ -393,7 +396,9 @@ int b200moe_block_norm(const b200moe_norm *norm, const void *x, const void *resi
 /*
  * Gated activation: x [M] rows of 2 I elements (gate, then linear), y [M, I] of the same type, or e4m3 with y_scale
  * [M, ceil(I/128)].  activation: B200MOE_ACT_*; alpha and limit (<= 0: no clamps) belong to B200MOE_ACT_SWIGLU_OAI.
+ * I up to B200MOE_ACT_MAX_I.
  */
+#define B200MOE_ACT_MAX_I (65535 * 4096)
 int b200moe_gated_activation(const void *x, int64_t ldx, int dtype, int M, int I, int activation, float alpha, float limit,
                              void *y, float *y_scale, int flags, void *stream);
 
