@@ -166,8 +166,7 @@ int launch_act(const ActArgs& a, int activation, cudaStream_t stream) {
 
 }  // namespace
 
-int launch_gated_activation(const ActArgs& a, int activation, int dtype, int num_sms, cudaStream_t stream) {
-  (void)num_sms;
+int launch_gated_activation(const ActArgs& a, int activation, int dtype, cudaStream_t stream) {
   switch (dtype) {
     case B200MOE_DTYPE_BF16: return launch_act<__nv_bfloat16>(a, activation, stream);
     case B200MOE_DTYPE_FP16: return launch_act<__half>(a, activation, stream);

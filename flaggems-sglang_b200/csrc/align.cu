@@ -2,6 +2,7 @@
 // expert with warp-match ranking and shared-memory counters.  Integer work only;
 // every output is deterministic (no atomics decide an order).
 #include "align.cuh"
+#include "cluster.cuh"
 
 namespace b200moe {
 
@@ -59,19 +60,10 @@ __device__ __forceinline__ int upper_expert(const int* offs, int n, int x) {
 // [c * per, (c + 1) * per), the CTAs' counts meet through distributed shared memory, and stability follows from
 // ordering by (CTA, warp, lane).  One CTA pushed every store through one SM's memory pipe (77 us at 32768 slots), and
 // two launches of 32 CTAs with the counts in global memory took 47 us there.
-__device__ __forceinline__ int cluster_rank() {
-  int r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // the int at this CTA's shared-memory address `p`, read in CTA `rank` of the cluster
 __device__ __forceinline__ int ld_cluster(const int* p, int rank) {
-  uint32_t a;
   int v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(mapa_u32(smem_u32(p), rank)) : "memory");
   return v;
 }
 
@@ -107,7 +99,7 @@ __device__ __forceinline__ void group_by_expert(const void* ids, int is64, const
                                                 int block, const GroupSmem& g, int nwarps, const float* pre, Place place,
                                                 int* dropped = nullptr) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int rank = cluster_rank(), nctas = gridDim.x;
+  const int rank = static_cast<int>(cluster_ctarank()), nctas = gridDim.x;
   for (int i = threadIdx.x; i < nwarps * E; i += blockDim.x) g.cnt[i] = 0;
   __syncthreads();
 
@@ -236,7 +228,7 @@ align_block_kernel(const void* ids, int is64, const int* map, int map_len, const
 
   // padding of every expert's group, then the unused tail of the tables
   const int lane = threadIdx.x & 31;
-  const int tid = cluster_rank() * blockDim.x + threadIdx.x, nthreads = gridDim.x * blockDim.x;
+  const int tid = static_cast<int>(cluster_ctarank()) * blockDim.x + threadIdx.x, nthreads = gridDim.x * blockDim.x;
   const int rows = g.base[E];
   for (int e = tid >> 5; e < E; e += nthreads >> 5)
     for (int r = g.base[e] + g.hist[e] + lane; r < g.base[e + 1]; r += 32) {
@@ -338,7 +330,7 @@ routing_from_topk_kernel(const float* weights, const void* ids, int is64, int M,
     }
     return t0 + rank;
   };
-  const int crank = cluster_rank(), nctas = gridDim.x;
+  const int crank = static_cast<int>(cluster_ctarank()), nctas = gridDim.x;
   const int tid = crank * blockDim.x + threadIdx.x, nthreads = nctas * blockDim.x;
   for (int i = tid; i < P; i += nthreads) expt_indx[sorted_slot(i)] = load_id(ids, is64, i);
 

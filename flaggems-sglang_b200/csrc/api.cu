@@ -1384,7 +1384,7 @@ int b200moe_gated_activation(const void* x, int64_t ldx, int dtype, int M, int I
   a.vec = I % 8 == 0 && rows_aligned(x, ldx, dtype_bytes(dtype), 16) && rows_aligned(y, 0, 1, y_scale ? 8 : 16);
   a.pdl = (flags & B200MOE_FLAG_NO_PDL) == 0;
   launch_log_new_call();
-  return launch_gated_activation(a, activation, dtype, query_sms(nullptr), static_cast<cudaStream_t>(stream));
+  return launch_gated_activation(a, activation, dtype, static_cast<cudaStream_t>(stream));
 }
 
 static int linear_args(const b200moe_linear* p, LinearArgs* a) {

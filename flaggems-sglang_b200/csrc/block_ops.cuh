@@ -5,8 +5,6 @@
 
 namespace b200moe {
 
-constexpr int kNormMaxH = 16384;
-
 struct NormArgs {
   const void* x;
   const void* residual;         // or null
@@ -39,7 +37,7 @@ struct ActArgs {
   float alpha, limit;           // B200MOE_ACT_SWIGLU_OAI; limit <= 0: no clamps
   int vec, pdl;
 };
-int launch_gated_activation(const ActArgs& a, int activation, int dtype, int num_sms, cudaStream_t stream);
+int launch_gated_activation(const ActArgs& a, int activation, int dtype, cudaStream_t stream);
 
 struct LinearArgs {
   int M, N, K, G;               // G = ceil(K / 128)
