@@ -1,11 +1,12 @@
 // Gated activation of [M, 2I] rows (gate, then linear), its result in the rows' type or quantised to e4m3 per 1 x 128 group.
 //
 //   silu        y = g / (1 + exp(-g)) * u
-//   gelu        y = g / 2 * (1 + erf(g / sqrt 2)) * u
+//   gelu        y = g Phi(g) u,  Phi the normal distribution
 //   swiglu_oai  g clamped from above, u to [-limit, limit];  y = g / (1 + exp(-alpha g)) * (u + 1)
 //
 // y is fp32 until it is rounded once, to its type or to e4m3.  Bound by HBM: 4 bytes in and 2 (or 1 + 1/32) out per
-// element; 4096 rows of 18432, silu, in 67.8 us (6.7 TB/s), quantised in 64.4 (5.9 TB/s, 90 % of a copy's rate).
+// element; 4096 rows of 18432, silu, in 68.0 us (6.7 TB/s), quantised in 64.6 (5.9 TB/s, 90 % of a copy's rate), swiglu_oai in 70.4 and 78.2.  GELU
+// is bound by its instructions: 85.1 and 93.3.
 // A thread takes two chunks of eight columns of a row; sixteen neighbours (rows off 16 bytes: a warp) hold a
 // group, so its maximum is found by shuffles.
 // Rows along the grid's x: no index needs a division.
@@ -30,11 +31,11 @@ __device__ __forceinline__ float rcp_fast(float x) {
 }
 __device__ __forceinline__ unsigned long long both(float v) { return pack_f32x2(v, v); }
 
-// exp(-a), exp(-b) for a, b in [0, 128]: 2^(-a log2 e) with what the product's rounding and that of log2 e leave, t = h + l, put back as
-// 2^h (1 + l ln 2).  (2^h alone is off by a 2^-24: 2^-19 of the result where a is 32.)
+// exp(-a), exp(-b) for a, b in [0, 128].  The exponent -a log2 e is -h + l: h the rounded product, l what its rounding and that of log2 e leave,
+// put back as 2^-h (1 + l ln 2).  (2^-h alone is off by a 2^-24: 2^-19 of the result where a is 32.)
 __device__ __forceinline__ unsigned long long exp_neg2(float a, float b) {
   constexpr float kHigh = 1.44269502162933349609375f, kLow = 1.92596299e-8f;      // log2 e
-  const unsigned long long x = pack_f32x2(a, b), h = mul2(x, both(kHigh));        // (h and l with their signs turned)
+  const unsigned long long x = pack_f32x2(a, b), h = mul2(x, both(kHigh));
   const unsigned long long l = fma2(x, both(-kLow), fma2(x, both(-kHigh), h));
   float ha, hb;
   unpack_f32x2(h, ha, hb);
@@ -51,7 +52,7 @@ __device__ __forceinline__ unsigned long long activate2(float g0, float g1, floa
   if (ACT == B200MOE_ACT_GELU) {
     // (max(g, 0) - a Phi(-a)) u with a = |g| and Phi(-a) = exp(-a^2 / 2) t P(t), t = 1 / (1 + 0.306 a): P is a polynomial of degree seven, fitted
     // to the least relative error over [0, 15], 2^-23.2 (in fp32 2^-21.2 at most, 2^-23.2 in the mean).  Relative to the result, so that
-    // negative g keep their digits: from 1 + erf(g / sqrt 2) they lose all of them down to -5, and erff takes 118 us where this takes 94,
+    // negative g keep their digits: from 1 + erf(g / sqrt 2) they lose all of them down to -5, and erff takes 118 us where this takes 93,
     // 4096 rows of 18432, quantised.  fp32 rows put the roundings of a^2 and of its product with log2 e / 2 back behind the exponential, as
     // above; for others they are a^2 2^-24 of a small result.
     constexpr float kHigh = 0.721347510814666748046875f, kLow = 9.62981495e-9f;        // log2 e / 2

@@ -70,7 +70,7 @@ linear_quant_kernel(const T* x, long long ldx, uint8_t* q, float* scales, int K,
 // ---------------------------------------------------------------- few rows: weights on the MMA's M side
 // A CTA takes 128 weight rows, NT tokens and a share of the reduction; the CTAs of a cluster share a tile's reduction and join
 // their sums through distributed shared memory, in rank order.
-// Bound by a launch's fixed way, then by memory: one row on 4096 x K takes 4.6 us at K = 896, 5.6 at 1792, 8.9 at 7168 (29.4 MB, 3.3 TB/s;
+// Bound by a launch's fixed way, then by memory: one row on 4096 x K takes 4.6 us at K = 896, 5.6 at 1792, 8.6 at 7168 (29.4 MB, 3.4 TB/s;
 // 4.5 us at the rate of a copy) and 22.1 at 28672 (117 MB, 5.3 TB/s).  Hence a ring as deep as half an SM's shared memory allows, two
 // CTAs to an SM, weights asked for in L2 ahead of the wait for the kernel before, and the reduction split over a cluster.
 struct DecodeSmem {

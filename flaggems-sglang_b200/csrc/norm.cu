@@ -11,10 +11,10 @@
 // mean's own rounding left there is taken off both, so rows with a large mean lose nothing.
 // Sums: shuffles within a warp, then one exchange through shared memory, always in the same order.
 //
-// Bound by HBM where there are many rows (of a copy's 6.54 TB/s): before a block, 4096 x 7168 quantised, 206.5 MB in 35.0 us, 90 %; after
-// a block, 8192 x 5120 with a gate per token, 251.7 MB in 40.3 us, 96 %; 2000 x 16384, 43.9 us, 91 %.  Two norms in one pass hold the
-// rows through four round trips of sums and reach 60 % (4096 x 4096, quantised, 30.2 us).  By a launch and one round trip to memory where
-// there are few: one row of 7168 in 2.6 us, 33 of 4096 with both norms in 3.2.
+// Bound by HBM where there are many rows (of a copy's 6.54 TB/s): before a block, 4096 x 7168 quantised, 206.5 MB in 35.8 us, 88 %; after
+// a block, 8192 x 5120 with a gate per token, 251.7 MB in 40.4 us, 95 %; 2000 x 16384, 43.9 us, 91 %.  Two norms in one pass hold the
+// rows through four round trips of sums and reach 60 % (4096 x 4096, quantised, 30.1 us).  By a launch and one round trip to memory where
+// there are few: one row of 7168 in 2.5 us, 33 of 4096 with both norms in 3.0.
 #include <algorithm>
 #include <type_traits>
 
@@ -619,6 +619,8 @@ int launch_rows(NormArgs a, int num_sms, cudaStream_t stream) {
   a.rows_per_cta = a.M > 2 * num_sms && a.team < 128 ? 128 / a.team : 1;
   const dim3 grid((a.M + a.rows_per_cta - 1) / a.rows_per_cta), block(a.team * a.rows_per_cta);
   note_launch("block_norm_kernel");
+  // Four chunks to a thread (rows of more than 8192 that the ring does not take: off 16 bytes, or fp32 beside their vectors) hold 128 registers and spill
+  // 8 to 184 bytes; a row is bound by its way from load to store all the same (2000 x 16384, fp32 residual, after a block 84.7 us).
   // A layer norm before a block needs a few registers more than the RMS norm; with 40 four of its CTAs of 352 threads share an SM, and three with
   // more (1001 x 2600, fp16: 7.3 us and 9.1).  Rows of 16-bit types fit into 40 without spills.
   constexpr bool SLIM = VEC && sizeof(T) == 2 && sizeof(R) == 2;

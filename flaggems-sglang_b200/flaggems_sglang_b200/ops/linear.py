@@ -87,7 +87,7 @@ def fp8_block_linear(
     ``gated_activation`` return them with ``quantize=True``.  The sums are fp32 and rounded once, to ``out_dtype`` (default:
     the type of a 16-bit ``x``, else bfloat16; float32 is possible).  ``bias``: ``[N]``.
 
-    K is a multiple of 16 up to 65536, N is free, no rows are an empty result.  ``weight`` may have strided rows that start on
+    K is a multiple of 16 up to 65536, N and the rows up to 2^31 - 256, no rows are an empty result.  ``weight`` may have strided rows that start on
     16 bytes; rows of ``x`` that do not are copied.  A NaN or an infinity makes its own row of the result NaN and no other.
     Forward only: no gradient is recorded.  ``tile`` / ``split`` pick the kernel by hand (tuning aid)."""
     global _fast

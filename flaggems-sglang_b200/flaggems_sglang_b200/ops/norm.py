@@ -189,9 +189,10 @@ def norm_before_block(
 
     ``gate``: ``[H]`` per channel, ``[..., 1]`` per token or ``[..., H]``.  ``residual`` has x's type or float32, and ``hidden`` has
     the residual's; ``inplace`` writes ``hidden`` over ``residual`` (x and residual are then the same rows or share none, and
-    neither gate nor vectors share memory with residual).  Without residual, gate and scale ``hidden`` is ``x`` itself.  All arithmetic is fp32; ``y`` is taken from ``hidden`` before that is
-    rounded.  Vectors and gate have x's type or float32; ``weight=None`` is a norm without weights.  H up to 16384; a 1-D gate of
-    H elements is per channel whatever the number of rows.  A NaN or an infinity concerns its own row only
+    neither gate nor vectors share memory with residual).  Without residual, gate and scale ``hidden`` is ``x`` itself.  All
+    arithmetic is fp32; ``y`` is taken from ``hidden`` before that is rounded; a layer norm's rows may have a mean that is large against their
+    deviation.  Vectors and gate have x's type or float32; ``weight=None`` is a norm without weights.  H up to 16384, rows up to 2^30;
+    a 1-D gate of H elements is per channel whatever the number of rows.  A NaN or an infinity concerns its own row only
     (quantised: a group's scale is that of its numbers, its values are what the formula gives).  Forward only: no gradient is recorded."""
     return _block_norm(x, False, True, None, None, weight, bias, residual, gate, residual_scale, eps, kind, weight_offset,
                        bool(quantize), bool(inplace))
