@@ -100,7 +100,8 @@ def _status_word(dev: torch.device) -> torch.Tensor:
                 rc = _lib.lib().b200moe_status_alloc(C.byref(word))
             if rc != _lib.OK:
                 _lib.check(rc, "status_alloc")
-            st = _status.setdefault(dev.index, torch.as_tensor(_DeviceWord(word.value), device=dev))
+            with torch.inference_mode(False):       # (a tensor made in inference mode could be cleared in that mode only)
+                st = _status.setdefault(dev.index, torch.as_tensor(_DeviceWord(word.value), device=dev))
     return st
 
 
@@ -118,7 +119,8 @@ def _deferred_status_check(dev: torch.device, status: torch.Tensor) -> None:
     idx = dev.index
     host = _status_host.get(idx)
     if host is None:
-        pinned = torch.zeros(1, dtype=torch.int32).pin_memory()
+        with torch.inference_mode(False):
+            pinned = torch.zeros(1, dtype=torch.int32).pin_memory()
         _status_host[idx] = host = (pinned, C.c_int.from_address(pinned.data_ptr()))
         _status_calls[idx] = 0
     elif host[1].value != 0 and not _capturing():   # plain host read: whatever an earlier copy has delivered
