@@ -5,8 +5,8 @@
 //   swiglu_oai  g clamped from above, u to [-limit, limit];  y = g / (1 + exp(-alpha g)) * (u + 1)
 //
 // y is fp32 until it is rounded once, to its type or to e4m3.  Bound by HBM: 4 bytes in and 2 (or 1 + 1/32) out per
-// element; 4096 rows of 18432, silu, in 68.0 us (6.7 TB/s), quantised in 64.6 (5.9 TB/s, 90 % of a copy's rate), swiglu_oai in 70.4 and 78.2.  GELU
-// is bound by its instructions: 85.1 and 93.3.
+// element; 4096 rows of 18432, silu, in 67.2 us (6.7 TB/s), quantised in 63.3 (6.0 TB/s, 92 % of a copy's rate), swiglu_oai in 74.3 and 77.4.  GELU
+// is bound by its instructions: 77.6 and 82.3.
 // A thread takes two chunks of eight columns of a row; sixteen neighbours (rows off 16 bytes: a warp) hold a
 // group, so its maximum is found by shuffles.
 // Rows along the grid's x: no index needs a division.
@@ -46,13 +46,13 @@ __device__ __forceinline__ unsigned long long exp_neg2(float a, float b) {
 // Two columns at once (packed fp32: what does not have to go through the special functions costs one instruction for both).
 // EXACT: fp32 rows.  Their results show what 16-bit ones and e4m3 round away (within 2^-24 (8 + |z|) of the result; over normally distributed rows
 // as few e4m3 values lie on the other side of a boundary either way), and their loads and stores take longer than the arithmetic:
-// 16-bit rows of 4096 x 18432, quantised, took 90 us this way and take 65 without.
+// 16-bit rows of 4096 x 18432, quantised, take 80 us this way and 63 without.
 template <int ACT, bool EXACT>
 __device__ __forceinline__ unsigned long long activate2(float g0, float g1, float u0, float u1, float alpha, float limit) {
   if (ACT == B200MOE_ACT_GELU) {
     // (max(g, 0) - a Phi(-a)) u with a = |g| and Phi(-a) = exp(-a^2 / 2) t P(t), t = 1 / (1 + 0.306 a): P is a polynomial of degree seven, fitted
     // to the least relative error over [0, 15], 2^-23.2 (in fp32 2^-21.2 at most, 2^-23.2 in the mean).  Relative to the result, so that
-    // negative g keep their digits: from 1 + erf(g / sqrt 2) they lose all of them down to -5, and erff takes 118 us where this takes 93,
+    // negative g keep their digits: from 1 + erf(g / sqrt 2) they lose all of them down to -5, and erff takes 104 us where this takes 82,
     // 4096 rows of 18432, quantised.  fp32 rows put the roundings of a^2 and of its product with log2 e / 2 back behind the exponential, as
     // above; for others they are a^2 2^-24 of a small result.
     constexpr float kHigh = 0.721347510814666748046875f, kLow = 9.62981495e-9f;        // log2 e / 2
@@ -127,7 +127,9 @@ gated_activation_kernel(const ActArgs a) {
   }
 #pragma unroll
   for (int r = 0; r < kRuns; ++r) {
-    // (whole warps stay: the shuffles below are the warp's)
+    // Whole warps stay: the shuffles below are the warp's.  One whose chunks all lie beyond the row leaves: half of the last CTA's of a row of
+    // 18432, and GELU took 94 us with their arithmetic and takes 82 without.
+    if ((first + r * static_cast<int>(blockDim.x) - lane) * 8 >= a.I) break;
     int e0, n;
     chunk_at<VEC>(first + r * blockDim.x, lane, a.I, e0, n);
     float g[8], u[8];
